@@ -37,8 +37,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// Running maximum of some z and the sum of 2^((z - maximum) c) over them.  The difference comes first where the maximum
-// times c is no number: of a row that holds nothing but the type's lowest value every column is as likely as any other.
+// Running maximum of some z and the sum of 2^((z - maximum) c) over them.
 struct Stat {
     float m, s;
 };
@@ -56,6 +55,23 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
     const float m = fmaxf(a.m, b.m), base = base_of(m);
     return {m, a.s * exp2f((a.m - base) * c) + b.s * exp2f((b.m - base) * c)};
 }
+// 2^((z - base) c) of many z.  The difference first would be two instructions and an exponent; z c + shift, shift = -base c, is
+// one, but off by shift's rounding, which grows with the row's distance from zero and which a softmax must not depend on (100
+// equal columns of 1e6 would sum to 101.5, of -1e30 to infinity).  What the rounding has taken away is a number that a fused
+// multiplication gives exactly, and as it is the same for all of a row's z, its power multiplies their sum, or whatever else
+// they are multiplied by.  From 2^20 on (masks of the lowest values) the difference comes first, as everywhere else.
+// (4096 x 60000 bfloat16 with gradient and rest: 210 us, and 223 with the difference first.)
+struct Powers {
+    float base, c, shift, more;
+    bool fused;
+    __device__ __forceinline__ Powers(float b, float by) : base(b), c(by), shift(-b * by) {
+        fused = fabsf(shift) <= 1048576.0f;
+        more = fused ? exp2f(fmaf(-b, by, -shift)) : 1.0f;
+    }
+    __device__ __forceinline__ float near(float z) const { return exp2_of(fmaf(z, c, shift)); }  // times more, where fused
+    __device__ __forceinline__ float far(float z) const { return exp2_of((z - base) * c); }
+};
+
 // Over all threads.  scratch: an entry a wave; a barrier has to lie between its last use and this.
 template <int kThreads>
 __device__ __forceinline__ float max_all(float v, float *scratch) {
@@ -128,23 +144,23 @@ struct Held {
     __device__ __forceinline__ float sum(float base, float c) {
         keep_packed();
         float s[4] = {};
-        const float shift = -base * c;
-        if (fabsf(shift) < __builtin_inff()) {
+        const Powers power(base, c);
+        if (power.fused) {
 #pragma unroll
             for (int h = 0; h < kHeld; ++h)
 #pragma unroll
-                for (int j = 0; j < kVec<T>; ++j) s[j % 4] += exp2_of(fmaf(v[h][j], c, shift));
-        } else {  // (nothing but the lowest values, or infinity)
+                for (int j = 0; j < kVec<T>; ++j) s[j % 4] += power.near(v[h][j]);
+        } else {  // (far from zero, or infinity)
 #pragma unroll 1
             for (int h = 0; h < kHeld; ++h) {
                 Vec<T> w = v[0];
 #pragma unroll
                 for (int i = 1; i < kHeld; ++i) w.raw = h == i ? v[i].raw : w.raw;
 #pragma unroll
-                for (int j = 0; j < kVec<T>; ++j) s[j % 4] += exp2_of((w[j] - base) * c);
+                for (int j = 0; j < kVec<T>; ++j) s[j % 4] += power.far(w[j]);
             }
         }
-        return (s[0] + s[1]) + (s[2] + s[3]);
+        return ((s[0] + s[1]) + (s[2] + s[3])) * power.more;
     }
 };
 
@@ -647,19 +663,19 @@ __device__ __forceinline__ void take_out(Held<T, kThreads, kHeld> &held, const u
 template <typename T, int kThreads, int kHeld>
 __device__ __forceinline__ void write_gradient(Held<T, kThreads, kHeld> &held, const Parts &r, float c, T *g, int n) {
     held.keep_packed();
-    const float factor = r.scale * r.factor, shift = -r.out_base * c;
-    const bool plain = fabsf(shift) < __builtin_inff();
+    const Powers power(r.out_base, c);
+    const float factor = r.scale * r.factor * power.more;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
         const int i = held.place(h);
         if (i >= n) break;
         float w[kVec<T>];
-        if (plain) {
+        if (power.fused) {
 #pragma unroll
-            for (int j = 0; j < kVec<T>; ++j) w[j] = factor * exp2_of(fmaf(held.v[h][j], c, shift));
+            for (int j = 0; j < kVec<T>; ++j) w[j] = factor * power.near(held.v[h][j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < kVec<T>; ++j) w[j] = factor * exp2_of((held.v[h][j] - r.out_base) * c);
+            for (int j = 0; j < kVec<T>; ++j) w[j] = factor * power.far(held.v[h][j]);
         }
         if (i + kVec<T> <= n) {
             store_vec(g + i, w);
