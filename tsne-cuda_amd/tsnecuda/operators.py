@@ -6,13 +6,16 @@ Arguments and results are torch CUDA tensors.  Every call only enqueues work on
 the current stream of its arguments' device; workspaces come from torch's
 allocator, on that stream.  Arguments that the library cannot take raise
 ``ValueError`` (``TypeError`` for what is no tensor of a supported type); a call
-that fails raises ``RuntimeError`` with the library's message.
+that fails raises ``RuntimeError`` with the library's message.  What a call
+writes into a tensor that it is given, autograd is told of, as of torch's own
+operations in place.
 """
 import collections
 import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import stages
 
@@ -216,6 +219,7 @@ def matmul_blocks(a, b, out_dtype=torch.bfloat16, out=None, exact=False):
     device = a._device
     if k != kb or device != b._device:
         raise ValueError("matmul_blocks: factors of %s and %s on %s and %s" % (a.shape, b.shape, a.device, b.device))
+    given = out
     out, stride = _result(out, m, n, out_dtype, device, "matmul_blocks")
     kind = _TYPES[out.dtype]
     lib = _lib()
@@ -223,6 +227,8 @@ def matmul_blocks(a, b, out_dtype=torch.bfloat16, out=None, exact=False):
     space = _workspace(size, device)
     _call(lib.tsne_hip_matmul_blocks, device.index, *a._pointers, *b._pointers, m, n, k, out.data_ptr(), kind, stride,
           1 if exact else 0, _ptr(space), size)
+    if given is not None:
+        increment_version(given)
     return out
 
 
@@ -340,6 +346,8 @@ def _distill(logits, indices, values, lse, weights, temperature, rest, want_grad
     _call(lib.tsne_hip_distill, device.index, logits.data_ptr(), kind, rows, cols, stride, indices.data_ptr(),
           values.data_ptr(), k, _ptr(lse), _ptr(weights), temperature, 1 if rest else 0, loss.data_ptr(), _ptr(grad),
           grad_stride, _ptr(space), size)
+    if out is not None:
+        increment_version(out)
     return loss, grad
 
 
