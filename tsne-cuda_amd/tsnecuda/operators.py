@@ -248,10 +248,14 @@ def linear_blocks(x, weight):
     """x (m x k) through a layer with BlockScaled weight (n x k): x is quantised
     and multiplied, in one call, into a result of x's type.  What a trained
     encoder places points with; the bits are those of
-    matmul_blocks(quantize_blocks(x), weight, x.dtype)."""
+    matmul_blocks(quantize_blocks(x), weight, x.dtype).  It has no gradient, and
+    where autograd would ask x for one it is refused."""
     if not isinstance(weight, BlockScaled):
         raise TypeError("linear_blocks: weight must be BlockScaled")
     x, m, k, stride = _rows(x, "linear_blocks", "x")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("linear_blocks has no gradient, and x requires one: block_linear has, and torch.no_grad() or x.detach() "
+                         "say that none is wanted")
     n, device = weight.shape[0], x.device
     if k != weight.shape[1] or device != weight._device:
         raise ValueError("linear_blocks: x of %s on %s and a weight of %s on %s" % (tuple(x.shape), device, weight.shape, weight.device))
