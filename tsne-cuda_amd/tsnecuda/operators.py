@@ -376,7 +376,12 @@ def distill_loss(logits, indices, values, lse=None, weights=None, temperature=1.
     list (columns, logits, and ln sum exp of the teacher's row at the same
     temperature; without lse the list's probabilities are made to sum to 1),
     times the row's weight.  With rest what the list leaves out counts as one
-    event.  Differentiable by the logits."""
+    event.  Differentiable by the logits, and by nothing else: a teacher or a
+    weight that wants a gradient is refused."""
+    if torch.is_grad_enabled():
+        for name, t in (("values", values), ("lse", lse), ("weights", weights)):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise ValueError("distill_loss: %s require a gradient, and there is none but the logits': detach them" % name)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return _Distill.apply(logits, indices, values, lse, weights, temperature, rest)
     return _distill(logits, indices, values, lse, weights, temperature, rest, False, None, "distill_loss")[0]
