@@ -139,13 +139,17 @@ class BlockScaled(object):
     def empty(cls, rows, cols, device):
         # (Both in one allocation, and no tensor made of either before somebody asks for it: each would cost a call as much
         # as a small kernel takes.)
+        size = rows * (_padded(cols, 128) + _padded(cols, 512) // 128)
+        return cls._of(torch.empty(size, dtype=torch.float8_e4m3fn, device=device), rows, cols)
+
+    @classmethod
+    def _of(cls, buffer, rows, cols):
+        """The matrix whose data and scales are one allocation."""
         made = cls.__new__(cls)
-        size = rows * _padded(cols, 128)
-        made._buffer = torch.empty(size + rows * (_padded(cols, 512) // 128), dtype=torch.float8_e4m3fn, device=device)
-        at = made._buffer.data_ptr()
-        made._pointers = at, at + size
+        at = buffer.data_ptr()
+        made._buffer, made._pointers = buffer, (at, at + rows * _padded(cols, 128))
         made._data = made._scales = None
-        made._device = made._buffer.device
+        made._device = buffer.device
         made.shape = rows, cols
         return made
 
@@ -275,16 +279,25 @@ class _BlockLinear(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad
         xq, xt = _quantize(x, False, True, need_w, "block_linear")
         wq, wt = _quantize(weight, True, True, need_x, "block_linear")
-        ctx.xt, ctx.wt, ctx.types = xt, wt, (x.dtype, weight.dtype)
+        ctx.save_for_backward(xt and xt._buffer, wt and wt._buffer)
+        ctx.how = x.shape, weight.shape, x.dtype, weight.dtype
         return matmul_blocks(xq, wq, out_dtype=x.dtype)
+
+    @staticmethod
+    def _kept(buffer, rows, cols):
+        # (A saved tensor is what the hooks on it give back: whatever they do, the kernels read aligned rows.)
+        buffer = buffer.contiguous()
+        return BlockScaled._of(buffer.clone() if buffer.data_ptr() % 16 else buffer, rows, cols)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         need_x, need_w = ctx.needs_input_grad
+        xt, wt = ctx.saved_tensors
+        (t, k), (n, _), x_type, w_type = ctx.how
         dyq, dyt = _quantize(dy, False, need_x, need_w, "block_linear")
-        dx = matmul_blocks(dyq, ctx.wt, out_dtype=ctx.types[0]) if need_x else None
-        dw = matmul_blocks(dyt, ctx.xt, out_dtype=ctx.types[1]) if need_w else None
+        dx = matmul_blocks(dyq, _BlockLinear._kept(wt, k, n), out_dtype=x_type) if need_x else None
+        dw = matmul_blocks(dyt, _BlockLinear._kept(xt, k, t), out_dtype=w_type) if need_w else None
         return dx, dw
 
 
