@@ -308,6 +308,9 @@ def block_linear(x, weight):
     x, weight = _matrix(x, "block_linear", "x"), _matrix(weight, "block_linear", "weight")
     if x.shape[1] != weight.shape[1] or x.device != weight.device:
         raise ValueError("block_linear: x of %s on %s and a weight of %s on %s" % (tuple(x.shape), x.device, tuple(weight.shape), weight.device))
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):  # (nothing to keep)
+        return matmul_blocks(_quantize(x, False, True, False, "block_linear")[0],
+                             _quantize(weight, True, True, False, "block_linear")[0], out_dtype=x.dtype)
     return _BlockLinear.apply(x, weight)
 
 
