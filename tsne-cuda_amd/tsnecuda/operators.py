@@ -285,7 +285,11 @@ class _BlockLinear(torch.autograd.Function):
 
     @staticmethod
     def _kept(buffer, rows, cols):
-        # (A saved tensor is what the hooks on it give back: whatever they do, the kernels read aligned rows.)
+        # (A saved tensor is what the hooks on it give back: whatever they do, the kernels read aligned rows, and all of them.)
+        size = rows * (_padded(cols, 128) + _padded(cols, 512) // 128)
+        if buffer.dtype != torch.float8_e4m3fn or buffer.shape != (size,):
+            raise RuntimeError("block_linear: a hook has put %s of shape %s in the place of %d saved values"
+                               % (buffer.dtype, tuple(buffer.shape), size))
         buffer = buffer.contiguous()
         return BlockScaled._of(buffer.clone() if buffer.data_ptr() % 16 else buffer, rows, cols)
 
