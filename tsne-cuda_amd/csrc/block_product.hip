@@ -2,10 +2,11 @@
 //
 // The 8-bit matrix instructions take the scales themselves, so that a product of blocks is one instruction for 16 x 16
 // results and nothing is rescaled.  They add products in groups of eight and drop, in each, what lies more than 2^-13 below
-// the largest (the groups' sums are added in 32 bits): an error of up to 7 * 2^-13 of a product, 1.5e-5 of a result for
-// normally distributed factors.  That is less than half a unit of bfloat16 (2^-9) and more than half a unit of a half
-// (2^-11), so results in halves and floats are summed from exact products (kExact), and bfloat16 on request: values times
-// scales are bf16 numbers, and the bf16 instructions lose nothing, at half the rate.
+// the largest (the groups' sums are added in 32 bits).  What that comes to, of a result: 1.5e-5 for normally distributed
+// factors, a hundredth of a bfloat16's half unit (2^-9) and not of a half's (2^-11) or a float's; at most 7 * 2^-13 of the
+// sum of its groups' largest products, which is more than any half unit where those cancel.  So results in halves and floats
+// are summed from exact products (kExact), and bfloat16 where the caller asks for it: values times scales are bf16 numbers,
+// and the bf16 instructions lose nothing, at half the rate.
 //
 // What a product is bound by changes with its size, and so does its form (cut_of).  us (TFLOP/s) into bfloat16 by the 8-bit
 // instructions and into floats, exactly; alone the instructions reach 3890 TFLOP/s on normally distributed values, a library's

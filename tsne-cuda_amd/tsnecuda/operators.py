@@ -213,10 +213,12 @@ def quantize_blocks_both(x, square=False):
 
 
 def matmul_blocks(a, b, out_dtype=torch.bfloat16, out=None, exact=False):
-    """a (m x k) times the transpose of b (n x k), both BlockScaled.  A bfloat16
-    result is summed by the 8-bit matrix instructions (relative error about 2e-5
-    before its rounding), a half or float32 one, and with exact any, from exact
-    products at half the rate."""
+    """a (m x k) times the transpose of b (n x k), both BlockScaled.  A half or
+    float32 result, and with exact any, is summed in 32 bits from exact products.
+    A bfloat16 one is otherwise summed by the 8-bit matrix instructions, at twice
+    the rate: of every eight products they drop what lies 2^-13 below the largest,
+    which for normally distributed factors is 1.5e-5 of a result, a hundredth of its
+    rounding, and more than its rounding where large products cancel."""
     if not isinstance(a, BlockScaled) or not isinstance(b, BlockScaled):
         raise TypeError("matmul_blocks: both factors must be BlockScaled")
     (m, k), (n, kb) = a.shape, b.shape
@@ -248,12 +250,12 @@ def _result(out, m, n, dtype, device, who):
     return out, out.stride(0) if m > 1 else n
 
 
-def linear_blocks(x, weight):
+def linear_blocks(x, weight, exact=False):
     """x (m x k) through a layer with BlockScaled weight (n x k): x is quantised
     and multiplied, in one call, into a result of x's type.  What a trained
     encoder places points with; the bits are those of
-    matmul_blocks(quantize_blocks(x), weight, x.dtype).  It has no gradient, and
-    where autograd would ask x for one it is refused."""
+    matmul_blocks(quantize_blocks(x), weight, x.dtype, exact=exact).  It has no
+    gradient, and where autograd would ask x for one it is refused."""
     if not isinstance(weight, BlockScaled):
         raise TypeError("linear_blocks: weight must be BlockScaled")
     x, m, k, stride = _rows(x, "linear_blocks", "x")
@@ -263,6 +265,8 @@ def linear_blocks(x, weight):
     n, device = weight.shape[0], x.device
     if k != weight.shape[1] or device != weight._device:
         raise ValueError("linear_blocks: x of %s on %s and a weight of %s on %s" % (tuple(x.shape), device, weight.shape, weight.device))
+    if exact and x.dtype == torch.bfloat16:  # (the one type whose products are not exact anyway)
+        return matmul_blocks(_quantize(x, False, True, False, "linear_blocks")[0], weight, x.dtype, exact=True)
     kind = _TYPES[x.dtype]
     out = x.new_empty((m, n))
     lib = _lib()
@@ -275,13 +279,13 @@ def linear_blocks(x, weight):
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight):
-        need_x, need_w = ctx.needs_input_grad
+    def forward(ctx, x, weight, exact):
+        need_x, need_w, _ = ctx.needs_input_grad
         xq, xt = _quantize(x, False, True, need_w, "block_linear")
         wq, wt = _quantize(weight, True, True, need_x, "block_linear")
         ctx.save_for_backward(xt and xt._buffer, wt and wt._buffer)
-        ctx.how = x.shape, weight.shape, x.dtype, weight.dtype
-        return matmul_blocks(xq, wq, out_dtype=x.dtype)
+        ctx.how = x.shape, weight.shape, x.dtype, weight.dtype, exact
+        return matmul_blocks(xq, wq, out_dtype=x.dtype, exact=exact)
 
     @staticmethod
     def _kept(buffer, rows, cols):
@@ -296,26 +300,28 @@ class _BlockLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        need_x, need_w = ctx.needs_input_grad
+        need_x, need_w, _ = ctx.needs_input_grad
         xt, wt = ctx.saved_tensors
-        (t, k), (n, _), x_type, w_type = ctx.how
+        (t, k), (n, _), x_type, w_type, exact = ctx.how
         dyq, dyt = _quantize(dy, False, need_x, need_w, "block_linear")
-        dx = matmul_blocks(dyq, _BlockLinear._kept(wt, k, n), out_dtype=x_type) if need_x else None
-        dw = matmul_blocks(dyt, _BlockLinear._kept(xt, k, t), out_dtype=w_type) if need_w else None
-        return dx, dw
+        dx = matmul_blocks(dyq, _BlockLinear._kept(wt, k, n), out_dtype=x_type, exact=exact) if need_x else None
+        dw = matmul_blocks(dyt, _BlockLinear._kept(xt, k, t), out_dtype=w_type, exact=exact) if need_w else None
+        return dx, dw, None
 
 
-def block_linear(x, weight):
+def block_linear(x, weight, exact=False):
     """x times the transpose of weight, differentiable: all three products of a
     training step are of 8-bit operands (x and the output's gradient scaled by 128
-    values along what is summed over, the weights by squares)."""
+    values along what is summed over, the weights by squares).  The result and its
+    gradient are of x's type, the weight's gradient of the weight's, and each is
+    summed as matmul_blocks sums that type, with exact from exact products."""
     x, weight = _matrix(x, "block_linear", "x"), _matrix(weight, "block_linear", "weight")
     if x.shape[1] != weight.shape[1] or x.device != weight.device:
         raise ValueError("block_linear: x of %s on %s and a weight of %s on %s" % (tuple(x.shape), x.device, tuple(weight.shape), weight.device))
     if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):  # (nothing to keep)
         return matmul_blocks(_quantize(x, False, True, False, "block_linear")[0],
-                             _quantize(weight, True, True, False, "block_linear")[0], out_dtype=x.dtype)
-    return _BlockLinear.apply(x, weight)
+                             _quantize(weight, True, True, False, "block_linear")[0], out_dtype=x.dtype, exact=exact)
+    return _BlockLinear.apply(x, weight, exact)
 
 
 TopLogits = collections.namedtuple("TopLogits", "values indices lse")
