@@ -76,3 +76,19 @@ def test_the_same_seed_trains_the_same_map(fitted):
         maps[0].fit(X[:600], embedding[:500])
     with pytest.raises(ValueError, match="num_neighbors"):
         maps[0].fit(X[:10], embedding[:10])
+
+
+@pytest.mark.gpu
+def test_weights_are_rounded_once(monkeypatch):
+    """The encoder's float32 weights become 8-bit ones directly, in training and afterwards, and their gradients are float32."""
+    from tsnecuda import operators, synthetic
+    X = synthetic.gaussian_clusters(600, d=50, clusters=8, center_scale=3.0, seed=7)
+    embedding = synthetic.initial_embedding(600, seed=8)
+    seen, block_linear = [], operators.block_linear
+    monkeypatch.setattr(operators, "block_linear", lambda x, w: seen.append(w.dtype) or block_linear(x, w))
+    mapping = ParametricMap(hidden=(200, 130), num_neighbors=20, perplexity=5.0, n_epochs=2).fit(X, embedding)
+    assert set(seen) == {torch.float32}
+    for w, q in zip(mapping._weights, mapping._quantized):
+        want = operators.quantize_blocks(w.detach(), square=True)
+        assert torch.equal(q.data.view(torch.uint8), want.data.view(torch.uint8))
+        assert torch.equal(q.scales.view(torch.uint8), want.scales.view(torch.uint8))

@@ -4,10 +4,11 @@ t-SNE moves the points it is given; it has no place for a later one.
 ``ParametricMap`` learns one: an encoder whose distribution over the fitted
 points (``softmax`` of the logarithms of Student's kernel between where it puts
 a point and where they are) is distilled from the point's own neighbour
-probabilities.  The encoder's wide layers run on 8-bit products
-(``operators.block_linear`` in training, ``operators.linear_blocks`` on weights
-quantised once afterwards), the neighbours' probabilities are the teacher's
-list of ``operators.distill_loss``.
+probabilities.  The encoder's wide layers run on 8-bit products of bfloat16
+activations and float32 weights (``operators.block_linear`` in training, with
+float32 gradients of the weights, ``operators.linear_blocks`` on weights quantised
+once afterwards), the neighbours' probabilities are the teacher's list of
+``operators.distill_loss``.
 
     embedding = TSNE(...).fit_transform(X)
     mapping = ParametricMap().fit(X, embedding)
@@ -57,7 +58,7 @@ class ParametricMap(object):
 
     def _hidden(self, x):
         for w in self._weights:
-            x = torch.relu(operators.block_linear(x, w.to(torch.bfloat16)))
+            x = torch.relu(operators.block_linear(x, w))
         return x
 
     def _head(self, h):
@@ -121,7 +122,7 @@ class ParametricMap(object):
                     total += loss.detach() * rows.numel()
                 self.losses_.append(total / n)
             self.losses_ = [float(v) for v in self.losses_]
-            self._quantized = [operators.quantize_blocks(w.detach().to(torch.bfloat16), square=True) for w in self._weights]
+            self._quantized = [operators.quantize_blocks(w.detach(), square=True) for w in self._weights]
         return self
 
     def _check_fitted(self):
