@@ -92,3 +92,25 @@ def test_weights_are_rounded_once(monkeypatch):
         want = operators.quantize_blocks(w.detach(), square=True)
         assert torch.equal(q.data.view(torch.uint8), want.data.view(torch.uint8))
         assert torch.equal(q.scales.view(torch.uint8), want.scales.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_a_fit_that_fails_leaves_no_map(fitted, monkeypatch):
+    from tsnecuda import operators
+    X, embedding, _ = fitted
+    mapping = ParametricMap(hidden=(130,), num_neighbors=20, perplexity=5.0, n_epochs=1).fit(X[:600], embedding[:600])
+    with pytest.raises(ValueError, match="shape"):  # (refused before anything is done: the map stays)
+        mapping.fit(X[:600], embedding[:500])
+    assert mapping.transform(X[:3]).shape == (3, 2)
+
+    def fails(*args, **how):
+        raise RuntimeError("no memory")
+
+    monkeypatch.setattr(operators, "distill_loss", fails)
+    for which in (mapping, ParametricMap(hidden=(130,), num_neighbors=20, perplexity=5.0, n_epochs=1)):
+        with pytest.raises(RuntimeError, match="no memory"):
+            which.fit(X[:600], embedding[:600])
+        assert which.losses_ is None
+        for ask in (which.transform, which.neighbors):
+            with pytest.raises(ValueError, match="fit"):
+                ask(X[:3])

@@ -79,6 +79,7 @@ class ParametricMap(object):
             raise ValueError("the embedding of %d points must be of shape (%d, 2) (got %s)" % (n, n, tuple(embedding.shape)))
         if not self.num_neighbors <= n <= operators.MAX_DISTILLED:
             raise ValueError("fit takes num_neighbors (%d) to %d points (got %d)" % (self.num_neighbors, operators.MAX_DISTILLED, n))
+        self.losses_ = None  # (until there is a map again)
         with torch.cuda.device(self.device):
             # The teacher: what the fit's own stages say of the points.  (A point's own entry has probability 0.)
             indices, square = stages.knn(X, self.num_neighbors)
@@ -98,7 +99,7 @@ class ParametricMap(object):
                           * spread[:, None]).requires_grad_()
             self._bias = embedding.mean(0).clone().requires_grad_()
             optimiser = torch.optim.Adam(self._weights + [self._last, self._bias], lr=self.learning_rate)
-            self.losses_ = []
+            losses = []
             batches = -(-n // self.batch_size)
             for epoch in range(self.n_epochs):
                 order = torch.randperm(n, generator=g, device=self.device)
@@ -120,9 +121,9 @@ class ParametricMap(object):
                     optimiser.step()
                     optimiser.zero_grad(set_to_none=True)
                     total += loss.detach() * rows.numel()
-                self.losses_.append(total / n)
-            self.losses_ = [float(v) for v in self.losses_]
+                losses.append(total / n)
             self._quantized = [operators.quantize_blocks(w.detach(), square=True) for w in self._weights]
+            self.losses_ = [float(v) for v in losses]
         return self
 
     def _check_fitted(self):
