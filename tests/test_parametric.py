@@ -114,3 +114,23 @@ def test_a_fit_that_fails_leaves_no_map(fitted, monkeypatch):
         for ask in (which.transform, which.neighbors):
             with pytest.raises(ValueError, match="fit"):
                 ask(X[:3])
+
+
+@pytest.mark.gpu
+def test_neighbors_of_many_points_take_little_memory(fitted):
+    X, _, mapping = fitted
+    many = torch.from_numpy(np.tile(X, (30, 1))).cuda()  # 120,000 points by 3000 places: 1.4 GB of distances
+    mapping.neighbors(many[:100], k=5)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    p, i = mapping.neighbors(many, k=5)
+    taken = torch.cuda.max_memory_allocated() - before
+    assert p.shape == i.shape == (120000, 5)
+    # (the points and hidden values as bfloat16 and floats are 120,000 x 256 x a few bytes)
+    assert taken < 1 << 30, taken
+    for a in (0, 4000, 116000):
+        q, j = mapping.neighbors(many[a:a + 4000], k=5)
+        assert torch.allclose(p[a:a + 4000], q, rtol=0.05) and (i[a:a + 4000] == j).float().mean() > 0.95
+    empty = mapping.neighbors(many[:0], k=5)
+    assert empty[0].shape == empty[1].shape == (0, 5)

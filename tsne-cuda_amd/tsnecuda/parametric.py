@@ -21,6 +21,8 @@ import torch
 
 from . import operators, stages
 
+_MOST_DISTANCES = 1 << 25
+
 
 class ParametricMap(object):
     """Encoder from input space into a finished embedding.
@@ -151,6 +153,10 @@ class ParametricMap(object):
         shares of the map's own distribution that they hold."""
         self._check_fitted()
         with torch.cuda.device(self.device), torch.no_grad():
-            top = operators.top_logits(self._logits(self._place(X)), k)
-            p, i = torch.exp(top.values - top.lse[:, None]), top.indices
+            y = self._place(X)
+            # So many rows at a time that their distances to all fitted points are 128 MB.
+            rows = max(1, _MOST_DISTANCES // len(self._anchors))
+            tops = [operators.top_logits(self._logits(y[r:r + rows]), k) for r in range(0, max(1, len(y)), rows)]
+            p = torch.cat([torch.exp(top.values - top.lse[:, None]) for top in tops])
+            i = torch.cat([top.indices for top in tops])
         return (p, i) if isinstance(X, torch.Tensor) else (p.cpu().numpy(), i.cpu().numpy())
