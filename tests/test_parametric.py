@@ -134,3 +134,23 @@ def test_neighbors_of_many_points_take_little_memory(fitted):
         assert torch.allclose(p[a:a + 4000], q, rtol=0.05) and (i[a:a + 4000] == j).float().mean() > 0.95
     empty = mapping.neighbors(many[:0], k=5)
     assert empty[0].shape == empty[1].shape == (0, 5)
+
+
+@pytest.mark.gpu
+def test_a_map_is_its_own(fitted):
+    """What a caller does with the embedding afterwards, or wants gradients of, or has switched off, is nothing to the map."""
+    X, embedding, _ = fitted
+    how = dict(hidden=(130,), num_neighbors=20, perplexity=5.0, n_epochs=1)
+    places = torch.from_numpy(np.ascontiguousarray(embedding[:600])).cuda()
+    mapping = ParametricMap(**how).fit(X[:600], places)
+    p, i = mapping.neighbors(X[600:700], k=5)
+    places.zero_()
+    q, j = mapping.neighbors(X[600:700], k=5)
+    assert np.array_equal(p, q) and np.array_equal(i, j)
+    with torch.no_grad():
+        again = ParametricMap(**how).fit(X[:600], embedding[:600])
+    assert np.allclose(again.losses_, mapping.losses_, rtol=1e-4)
+    points = torch.from_numpy(X[:600].copy()).cuda().requires_grad_()
+    again = ParametricMap(**how).fit(points, embedding[:600])
+    assert points.grad is None and np.allclose(again.losses_, mapping.losses_, rtol=1e-4)
+    assert not again.transform(points).requires_grad

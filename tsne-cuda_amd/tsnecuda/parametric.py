@@ -53,7 +53,7 @@ class ParametricMap(object):
         X = torch.as_tensor(np.ascontiguousarray(X, dtype=np.float32) if not isinstance(X, torch.Tensor) else X)
         if X.dim() != 2:
             raise ValueError("points must be a matrix (got shape %s)" % (tuple(X.shape),))
-        return X.to(self.device, torch.float32).contiguous()
+        return X.detach().to(self.device, torch.float32).contiguous()
 
     def _scaled(self, X):
         return ((X - self._mean) * self._scale).to(torch.bfloat16)
@@ -82,12 +82,12 @@ class ParametricMap(object):
         if not self.num_neighbors <= n <= operators.MAX_DISTILLED:
             raise ValueError("fit takes num_neighbors (%d) to %d points (got %d)" % (self.num_neighbors, operators.MAX_DISTILLED, n))
         self.losses_ = None  # (until there is a map again)
-        with torch.cuda.device(self.device):
+        with torch.cuda.device(self.device), torch.enable_grad():
             # The teacher: what the fit's own stages say of the points.  (A point's own entry has probability 0.)
             indices, square = stages.knn(X, self.num_neighbors)
             pij = stages.perplexity(stages.max_normalize_(square), self.perplexity, self.perplexity_epsilon)
             values = torch.log(pij)
-            self._anchors = embedding
+            self._anchors = embedding.clone()
             self._mean = X.mean(0)
             self._scale = 1.0 / (X - self._mean).std().clamp(min=1e-30)
             x = self._scaled(X)
