@@ -616,7 +616,7 @@ __device__ __forceinline__ Parts make_parts(const Distill &d, const List &l, Sta
         pr = fmaxf(0.0f, 1.0f - mass);
         if (pr > 0.0f) part += pr * (logf(pr) - (ln_q(out.m) + logf(out.s)));
     }
-    if (loss && threadIdx.x == 0) *loss = w * part;
+    if (loss && threadIdx.x == 0) *loss = w * (all.s != all.s ? all.s : part);  // (no number, also where no p asks for one)
     // Outside the list q total - p_r q / q_r, from those columns' own maximum, so that nothing overflows where they are far
     // below the list's.  (Where nothing is finite out there every term is 0; a sum that is no number goes everywhere.)
     Parts r = {base, all.s, mass + pr, base_of(out.m), all.s != all.s ? all.s : 0.0f, w / d.temperature};
