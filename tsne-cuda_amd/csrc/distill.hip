@@ -292,10 +292,9 @@ __device__ __forceinline__ void clear_top(TopShared<kThreads> &sh) {
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
 }
-// From the k-th largest of the threads' keys on, after clear_top().  (With k > kThreads everything.)
+// From the k-th largest of the threads' keys on, after clear_top(); k is at most kThreads.
 template <int kThreads>
 __device__ __forceinline__ unsigned int threshold_of(TopShared<kThreads> &sh, int k, unsigned int key) {
-    if (k > kThreads) return 0;
     int want = k;
     atomicAdd(&first_counts(sh)[key >> 24], 1u);
     __syncthreads();
@@ -412,18 +411,14 @@ __global__ __launch_bounds__(kThreads, kHeld == 8 && kThreads > 256 ? 8 : 4) voi
     // threshold_of(), but that the barriers of the maximum and of the sum are its own too.
     const float my_max = held.max();
     const unsigned int key = key_of(my_max);
-    const bool by_threads = k <= kThreads;
-    unsigned int digit = 0, prefix = 0;
     int want = k;
-    if (by_threads) atomicAdd(&first_counts(sh)[key >> 24], 1u);
+    atomicAdd(&first_counts(sh)[key >> 24], 1u);
     Stat st = {max_all<kThreads>(my_max, sh.floats), 0.0f};
-    if (by_threads) {
-        digit = (unsigned int)find_digit(first_counts(sh), want);
-        if (key >> 24 == digit) atomicAdd(&sh.counts[key >> 16 & 255], 1u);
-    }
+    const unsigned int digit = (unsigned int)find_digit(first_counts(sh), want);
+    if (key >> 24 == digit) atomicAdd(&sh.counts[key >> 16 & 255], 1u);
     const float my_sum = held.sum(base_of(st.m), c);
     st.s = sum_all<kThreads>(my_sum, sh.sums);
-    if (by_threads) prefix = digit << 24 | (unsigned int)find_digit(sh.counts, want) << 16;
+    unsigned int prefix = digit << 24 | (unsigned int)find_digit(sh.counts, want) << 16;
     bool my_nan = false;
     if (st.s != st.s) {  // NaN, of which the maxima know nothing, or infinity
 #pragma unroll
@@ -861,6 +856,8 @@ Holding holding_of(int64_t cols, int type, bool many, int least_threads, bool in
 // unit can be held (1000 x 131072 floats: 450 us with stretches of 4096, 120 with 32768).
 int top_stretch(int64_t rows) { return rows <= kFewTopRows ? kStretch : 8 * kStretch; }
 
+// (The threshold is the k-th largest of the threads' maxima: there are k of them at least, 1024 in stretches.)
+static_assert(kWaveListed <= kWave && kGroupListed <= 256 && kMostListed <= 1024 && kMostListed <= kStretch);
 int top_threads(int k) { return k <= kWaveListed ? kWave : k <= kGroupListed ? 256 : 1024; }
 
 Holding top_holding(int64_t rows, int64_t cols, int type, int k) {
