@@ -884,13 +884,6 @@ int check_type(const char *who, int type) {
     return 0;
 }
 
-int check_workspace(const char *who, const void *workspace, int64_t bytes, int64_t needed) {
-    TSNE_OPERATOR_REQUIRE(bytes >= needed && (workspace || needed == 0), "%s: the workspace has %lld bytes and not %lld", who,
-                          (long long)bytes, (long long)needed);
-    TSNE_OPERATOR_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be aligned to 16 bytes", who);
-    return 0;
-}
-
 int check_product(const char *who, int64_t m, int64_t n, int64_t k, int64_t c_stride) {
     TSNE_OPERATOR_REQUIRE(m >= 0 && n >= 0 && k >= 0 && k <= kMostSummed, "%s: a product of %lld x %lld x %lld (at most %lld are summed)", who,
                           (long long)m, (long long)n, (long long)k, (long long)kMostSummed);

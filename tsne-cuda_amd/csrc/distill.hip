@@ -896,13 +896,6 @@ int by_holding(const Holding &h, F f) {
     return f(integral_constant<int, 1024>(), integral_constant<int, 16>());
 }
 
-int check_workspace(const char *who, const void *workspace, int64_t bytes, int64_t needed) {
-    TSNE_OPERATOR_REQUIRE(bytes >= needed && (workspace || needed == 0), "%s: the workspace has %lld bytes and not %lld", who,
-                          (long long)bytes, (long long)needed);
-    TSNE_OPERATOR_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be aligned to 16 bytes", who);
-    return 0;
-}
-
 }  // namespace
 }  // namespace tsnehip
 

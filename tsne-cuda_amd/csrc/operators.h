@@ -23,6 +23,13 @@ inline int64_t block_scale_stride(int64_t cols) { return (cols + 4 * kBlock - 1)
         }                                \
     } while (0)
 
+inline int check_workspace(const char *who, const void *workspace, int64_t bytes, int64_t needed) {
+    TSNE_OPERATOR_REQUIRE(bytes >= needed && (workspace || needed == 0), "%s: the workspace has %lld bytes and not %lld", who,
+                          (long long)bytes, (long long)needed);
+    TSNE_OPERATOR_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: the workspace must be aligned to 16 bytes", who);
+    return 0;
+}
+
 int launch_quantize(const void *x, int type, int64_t rows, int64_t cols, int64_t row_stride, int square, uint8_t *data,
                     uint8_t *scales, uint8_t *data_t, uint8_t *scales_t, hipStream_t s);
 
