@@ -372,7 +372,8 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void tiled_product_kernel(
             }
         };
         if constexpr (kExact && kFM * kFN > 16) {
-            // So many results leave no registers for a choice in every block: the wave looks at all its scales first.
+            // So many results leave no registers for a choice in every block: each wave looks at all its scales first, and
+            // as the ways that follow have barriers, all waves take the same.
             unsigned int least = 255, most = 0;
             for (int row = lane; row < 16 * (kFM + kFN); row += kWave) {
                 const bool of_a = row < 16 * kFM;
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(Shape::kThreads, 2) void tiled_product_kernel(
                     for (int q = 0; q < 4; ++q) least = min(least, four >> 8 * q & 255), most = max(most, four >> 8 * q & 255);
                 }
             }
-            if (__all(plain_scales(least, most))) {
+            if (__syncthreads_and(plain_scales(least, most))) {
                 all_blocks([&](const unsigned char *la, const unsigned char *lb) __attribute__((always_inline)) {
                     bf16x8 wb[kFN][4];
 #pragma unroll
