@@ -81,7 +81,8 @@ int64_t tsne_hip_top_logits_workspace(int64_t rows, int64_t cols, int type, int 
  * of q over the columns that are not listed, as one event; it is left out where every column outside the list is
  * -infinity.  A listed column with p_j = 0 adds nothing.  w = 0: loss and gradient are exactly 0 and the row's
  * logits are not looked at.
- * grad (type of the logits, may be NULL, may be the logits themselves) receives the derivative of loss[row] by z.
+ * grad (type of the logits, may be NULL, may be the logits themselves, but may not overlap them otherwise) receives the
+ * derivative of loss[row] by z.
  * A column that is -infinity has q = 0 and, unless it is listed, gradient 0: with p_j > 0 on it the loss is
  * +infinity and its gradient -w p_j / temperature.  NaN and +infinity in a row make its loss and gradient NaN.
  * 1 <= k <= 1024, cols <= 2^20, temperature > 0.  With perplexity's probabilities as the teacher: values = ln pij,

@@ -896,6 +896,19 @@ int by_holding(const Holding &h, F f) {
     return f(integral_constant<int, 1024>(), integral_constant<int, 16>());
 }
 
+// Whether a gradient has values where other logits are, so that what one workgroup reads another may have written.  (Rows of
+// both that are equally far apart may lie between one another; otherwise the two have to be apart.)
+bool overlap(const void *logits, int64_t row_stride, const void *grad, int64_t grad_stride, int64_t rows, int64_t cols, int type) {
+    const int64_t size = (int64_t)type_size(type);
+    const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(grad) - reinterpret_cast<uintptr_t>(logits));  // (bytes)
+    if (apart == 0) return false;
+    auto extent = [&](int64_t stride) { return ((rows - 1) * stride + cols) * size; };
+    if (apart >= extent(row_stride) || -apart >= extent(grad_stride)) return false;
+    if (rows == 1 || row_stride != grad_stride) return true;
+    const int64_t step = row_stride * size, within = (apart % step + step) % step;  // from a row of logits to the next gradient
+    return within < cols * size || within > step - cols * size;
+}
+
 }  // namespace
 }  // namespace tsnehip
 
@@ -976,6 +989,8 @@ extern "C" int tsne_hip_distill(const void *logits, int type, int64_t rows, int6
     TSNE_OPERATOR_REQUIRE(logits && indices && values && loss, "distill: null argument");
     TSNE_OPERATOR_REQUIRE(grad != logits || grad_stride == row_stride,
                           "distill: a gradient in the logits' place has to have their stride");
+    TSNE_OPERATOR_REQUIRE(!grad || !overlap(logits, row_stride, grad, grad_stride, rows, cols, type),
+                          "distill: the gradient overlaps the logits, and is not in their place");
     if (check_workspace("distill", workspace, workspace_bytes, tsne_hip_distill_workspace(rows, cols, type, k))) return 1;
     const hipStream_t s = (hipStream_t)stream;
     const Holding h = distill_holding(rows, cols, type);
