@@ -66,7 +66,7 @@ int64_t tsne_hip_linear_blocks_workspace(int64_t m, int64_t n, int64_t k, int ty
 /* For every row of logits its k largest (values, descending; equal ones by ascending column) and their columns,
  * and lse = ln sum exp(z / temperature) over the whole row, all in 32 bits.  A column that is -infinity is never
  * listed: where a row has fewer than k others, the rest of its list is (-infinity, -1).  NaN counts as the largest;
- * it and +infinity make the row's lse NaN.  A row of -infinity has lse = -infinity.  1 <= k <= min(cols, 1024), cols < 2^31, temperature > 0. */
+ * it and +infinity make the row's lse NaN.  A row of -infinity has lse = -infinity.  1 <= k <= min(cols, 1024), cols < 2^31, temperature from 2^-126 on. */
 int tsne_hip_top_logits(const void *logits, int type, int64_t rows, int64_t cols, int64_t row_stride, int k,
                         float temperature, float *values, int *indices, float *lse, void *workspace,
                         int64_t workspace_bytes, void *stream);
@@ -85,7 +85,7 @@ int64_t tsne_hip_top_logits_workspace(int64_t rows, int64_t cols, int type, int 
  * derivative of loss[row] by z.
  * A column that is -infinity has q = 0 and, unless it is listed, gradient 0: with p_j > 0 on it the loss is
  * +infinity and its gradient -w p_j / temperature.  NaN and +infinity in a row make its loss and gradient NaN.
- * 1 <= k <= 1024, cols <= 2^20, temperature > 0.  With perplexity's probabilities as the teacher: values = ln pij,
+ * 1 <= k <= 1024, cols <= 2^20, temperature from 2^-126 on.  With perplexity's probabilities as the teacher: values = ln pij,
  * lse = NULL, temperature = 1. */
 int tsne_hip_distill(const void *logits, int type, int64_t rows, int64_t cols, int64_t row_stride, const int *indices,
                      const float *values, int k, const float *lse, const float *weights, float temperature, int rest,

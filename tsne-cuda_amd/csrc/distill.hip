@@ -929,8 +929,7 @@ extern "C" int tsne_hip_top_logits(const void *logits, int type, int64_t rows, i
                           (long long)row_stride);
     TSNE_OPERATOR_REQUIRE(k >= 1 && k <= kMostListed && k <= cols, "top_logits: k must be in [1, min(%lld, %d)] (got %d)",
                           (long long)cols, kMostListed, k);
-    TSNE_OPERATOR_REQUIRE(temperature > 0.0f && temperature < __builtin_inff(),
-                          "top_logits: the temperature must be positive (got %g)", (double)temperature);
+    if (check_temperature("top_logits", temperature)) return 1;
     if (rows == 0) return 0;
     TSNE_OPERATOR_REQUIRE(logits && values && indices && lse, "top_logits: null argument");
     if (check_workspace("top_logits", workspace, workspace_bytes, tsne_hip_top_logits_workspace(rows, cols, type, k))) return 1;
@@ -981,8 +980,7 @@ extern "C" int tsne_hip_distill(const void *logits, int type, int64_t rows, int6
                           "distill: rows of %lld values are only %lld and %lld apart", (long long)cols,
                           (long long)row_stride, (long long)grad_stride);
     TSNE_OPERATOR_REQUIRE(k >= 1 && k <= kMostListed, "distill: k must be in [1, %d] (got %d)", kMostListed, k);
-    TSNE_OPERATOR_REQUIRE(temperature > 0.0f && temperature < __builtin_inff(),
-                          "distill: the temperature must be positive (got %g)", (double)temperature);
+    if (check_temperature("distill", temperature)) return 1;
     TSNE_OPERATOR_REQUIRE(rest == 0 || rest == 1, "distill: rest must be 0 or 1 (got %d)", rest);
     TSNE_OPERATOR_REQUIRE(rest == 0 || lse, "distill: rest needs the teacher's lse");
     if (rows == 0) return 0;

@@ -30,6 +30,13 @@ inline int check_workspace(const char *who, const void *workspace, int64_t bytes
     return 0;
 }
 
+// (Below 2^-126 its reciprocal is infinite, and a difference of nothing times that no number.)
+inline int check_temperature(const char *who, float temperature) {
+    TSNE_OPERATOR_REQUIRE(temperature >= 0x1p-126f && temperature < __builtin_inff(),
+                          "%s: the temperature must be positive, 2^-126 at least (got %g)", who, (double)temperature);
+    return 0;
+}
+
 int launch_quantize(const void *x, int type, int64_t rows, int64_t cols, int64_t row_stride, int square, uint8_t *data,
                     uint8_t *scales, uint8_t *data_t, uint8_t *scales_t, hipStream_t s);
 

@@ -23,6 +23,7 @@ _vp, _ci, _cf, _c64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_in
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_LISTED = 1024
 MAX_DISTILLED = 1 << 20
+_LEAST, _INFINITE = 2.0 ** -126, 2.0 ** 128 * (1 - 2.0 ** -25)  # (of temperatures, as floats hold them)
 
 _bound = None
 
@@ -330,12 +331,13 @@ TopLogits = collections.namedtuple("TopLogits", "values indices lse")
 def top_logits(logits, k, temperature=1.0):
     """A teacher's list: of every row the k largest logits (float32, descending,
     equal ones by ascending column), their columns (int32; -1 where a row has
-    fewer than k that are not -infinity) and ln sum exp(logits / temperature)."""
+    fewer than k that are not -infinity) and ln sum exp(logits / temperature).  A
+    teacher's list is a constant: no gradient goes through it."""
     logits, rows, cols, stride = _rows(logits, "top_logits", "logits")
     if not 1 <= k <= min(cols, MAX_LISTED):
         raise ValueError("top_logits: k must be in [1, %d] (got %s)" % (min(cols, MAX_LISTED), k))
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError("top_logits: the temperature must be positive (got %s)" % temperature)
+    if not _LEAST <= temperature < _INFINITE:
+        raise ValueError("top_logits: the temperature must be positive, as a float (got %s)" % temperature)
     device = logits.device
     values = torch.empty((rows, k), dtype=torch.float32, device=device)
     indices = torch.empty((rows, k), dtype=torch.int32, device=device)
@@ -361,8 +363,8 @@ def _distill(logits, indices, values, lse, weights, temperature, rest, want_grad
     values = _vector(values, (rows, k), torch.float32, device, who, "values")
     lse = None if lse is None else _vector(lse, (rows,), torch.float32, device, who, "lse")
     weights = None if weights is None else _vector(weights, (rows,), torch.float32, device, who, "weights")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError("%s: the temperature must be positive (got %s)" % (who, temperature))
+    if not _LEAST <= temperature < _INFINITE:
+        raise ValueError("%s: the temperature must be positive, as a float (got %s)" % (who, temperature))
     if rest and lse is None:
         raise ValueError("%s: rest needs the teacher's lse" % who)
     grad, grad_stride = _result(out, rows, cols, logits.dtype, device, who) if want_grad else (None, 0)
@@ -416,5 +418,6 @@ def distill_loss(logits, indices, values, lse=None, weights=None, temperature=1.
 def distill(logits, indices, values, lse=None, weights=None, temperature=1.0, rest=False, out=None):
     """(distill_loss, its gradient by the logits) in one pass, for training loops
     whose loss is the rows' sum: what each row's gradient is multiplied by goes into
-    weights.  out: where the gradient goes; the logits themselves are allowed."""
+    weights.  Neither is part of autograd's graph.  out: where the gradient goes; the
+    logits themselves are allowed, where no backward pass still needs them."""
     return _distill(logits, indices, values, lse, weights, temperature, rest, True, out, "distill")
