@@ -27,6 +27,9 @@ constexpr float kLog2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float lowest() { return -__builtin_inff(); }
 
+// (What all lanes hold alike: in a scalar register, of which there are enough.)
+__device__ __forceinline__ float uniform(float v) { return lane_value(v, 0); }
+
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // (0 below 2^-126)
 
 // (fmaxf adds a quieting move an operand.  A signalling NaN comes out as NaN here, a quiet one is passed over; the sums that
@@ -60,16 +63,14 @@ __device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
 // equal columns of 1e6 would sum to 101.5, of -1e30 to infinity).  What the rounding has taken away is a number that a fused
 // multiplication gives exactly, and as it is the same for all of a row's z, its power multiplies their sum, or whatever else
 // they are multiplied by.  From 2^20 on (masks of the lowest values) the difference comes first, as everywhere else.
-// (4096 x 60000 bfloat16 with gradient and rest: 210 us, and 223 with the difference first.)
+// (4096 x 60000 bfloat16 with gradient and rest, pass after pass: 210 us, and 223 with the difference first.)
 struct Powers {
-    float base, c, shift, more;
+    float base, c, shift;
     bool fused;
-    __device__ __forceinline__ Powers(float b, float by) : base(b), c(by), shift(-b * by) {
-        fused = fabsf(shift) <= 1048576.0f;
-        more = fused ? exp2f(fmaf(-b, by, -shift)) : 1.0f;
-    }
-    __device__ __forceinline__ float near(float z) const { return exp2_of(fmaf(z, c, shift)); }  // times more, where fused
+    __device__ __forceinline__ Powers(float b, float by) : base(uniform(b)), c(uniform(by)), shift(uniform(-b * by)), fused(fabsf(shift) <= 1048576.0f) {}
+    __device__ __forceinline__ float near(float z) const { return exp2_of(fmaf(z, c, shift)); }  // times more(), where fused
     __device__ __forceinline__ float far(float z) const { return exp2_of((z - base) * c); }
+    __device__ __forceinline__ float more() const { return exp2_of(fmaf(-base, c, -shift)); }  // (2^(1/16) at most)
 };
 
 // Over all threads.  scratch: an entry a wave; a barrier has to lie between its last use and this.
@@ -81,7 +82,7 @@ __device__ __forceinline__ float max_all(float v, float *scratch) {
     v = scratch[0];
 #pragma unroll
     for (int w = 1; w < kThreads / kWave; ++w) v = fmaxf(v, scratch[w]);
-    return v;
+    return uniform(v);
 }
 template <int kThreads>
 __device__ __forceinline__ float sum_all(float v, float *scratch) {
@@ -91,7 +92,7 @@ __device__ __forceinline__ float sum_all(float v, float *scratch) {
     v = scratch[0];
 #pragma unroll
     for (int w = 1; w < kThreads / kWave; ++w) v += scratch[w];
-    return v;
+    return uniform(v);
 }
 template <int kThreads>
 __device__ __forceinline__ Stat join_all(Stat v, float c, Stat *scratch) {
@@ -160,7 +161,8 @@ struct Held {
                 for (int j = 0; j < kVec<T>; ++j) s[j % 4] += power.far(w[j]);
             }
         }
-        return ((s[0] + s[1]) + (s[2] + s[3])) * power.more;
+        const float all = (s[0] + s[1]) + (s[2] + s[3]);
+        return power.fused ? all * power.more() : all;
     }
 };
 
@@ -659,7 +661,7 @@ template <typename T, int kThreads, int kHeld>
 __device__ __forceinline__ void write_gradient(Held<T, kThreads, kHeld> &held, const Parts &r, float c, T *g, int n) {
     held.keep_packed();
     const Powers power(r.out_base, c);
-    const float factor = r.scale * r.factor * power.more;
+    const float factor = uniform(r.scale * r.factor * (power.fused ? power.more() : 1.0f));
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
         const int i = held.place(h);
