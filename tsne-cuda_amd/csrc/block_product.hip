@@ -16,7 +16,7 @@
 //                                                                       64 KB of factors a block through each unit's load path
 //   128 x 128, two teams  4096 x 1024 x 8192     38 (1835)   68 (1014)  the same, for half the products a byte
 //   64 x 64, four teams   512 x 2048 x 4096      12 (710)    16 (551)   a block's way from memory through LDS, 1.2 us a step
-//   64 x 64               1203 x 1111 x 784       6 (333)     9 (223)   the first loads' latency
+//   64 x 64               1203 x 1111 x 784       6 (335)     9 (225)   the first loads' latency (7 on factors just written)
 //   16 rows               1 x 8192 x 8192        15          17         reading b, 4.4 TB/s (a copy runs at 4.8)
 #include "../../include/tsnecuda/tsne_operators.h"
 #include "lds_load.h"

@@ -6,11 +6,13 @@
 // at different stages, one loading while another computes or stores.  Few long rows, and rows beyond registers, are cut into
 // stretches whose results a second kernel joins.  us, and GB/s of what has to be moved (a copy's rate is 4785):
 //                            loss and gradient, rest   loss alone    top list
-//   4096 x 60000 bf16, k 90      216.9  4532           129.5  3794   133.5  3681   (reading alone: a large sum runs at 4012)
-//   2048 x 32003 bf16, k 45       66.6  3935            30.7  4265    37.5  3496
-//   4096 x 2000  bf16, k 45       13.2  2490             7.2  2265    15.2  1080   (the list's own work)
-//    600 x 1200  bf16, k 90        8.0                   5.3          13.0         (latency: loads, barriers, one list)
-//      7 x 131071 bf16, k 90      10.8                   7.8          15.1         (and a second launch's)
+//   4096 x 60000 bf16, k 90      217.8  4513           131.7  3732   131.5  3737   (reading alone: a large sum runs at 4012)
+//   2048 x 32003 bf16, k 45       67.3  3896            31.1  4214    36.6  3584
+//   4096 x 2000  bf16, k 45       13.4  2440             7.4  2211    15.4  1063   (the list's own work)
+//    600 x 1200  bf16, k 90        8.1                   5.4          13.2         (latency: loads, barriers, one list)
+//      7 x 131071 bf16, k 90      11.0                   8.1          15.2         (and a second launch's)
+//   1000 x 131072 f32, k 90      291.8  3593           105.3  4979                 (no rest; beyond registers, so that both kernels of
+//                                                                                  a gradient read the logits: 5390 of three transfers)
 #include <algorithm>
 #include <type_traits>
 

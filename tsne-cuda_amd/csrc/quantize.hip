@@ -7,7 +7,7 @@
 // everything.  A row's block is complete in the 16 threads that load it and is written at once; the values go to LDS as they
 // came, where eight threads find a column's (a word's two columns at a time) with 16 rows each.  Both orientations of
 // 8192 x 4096 bfloat16 27 us (5.0 TB/s; a copy runs at 4.8; 31 with the rows read from LDS again and a column at a time), of
-// 4096 x 4096 floats 20.1 (5.0; by squares 22.9); of 8195 x 1024 11.4 to 11.9 (2.9), where the tiles are too few to cover one
+// 4096 x 4096 floats 20.1 (5.0; by squares 22.9); of 8195 x 1024 11.5 to 12.4 (2.7 to 2.9), where the tiles are too few to cover one
 // another's loads, way through LDS and stores.
 #include "../../include/tsnecuda/tsne_operators.h"
 #include "operators.h"
